@@ -213,22 +213,7 @@ typedef __attribute__((address_space(1))) const int16_t* JxltGlobalConstShorts;
 typedef __attribute__((address_space(1))) const uint32_t* JxltGlobalConstWords;
 #endif
 
-// p[i] = v for a wave-uniform 64-bit value and a wave-uniform, 8-byte aligned address in global memory: ONE scalar
-// store (s_store_dwordx2; i: a compile-time index) instead of moves to vector registers and a vector store by one
-// lane.  Scalar stores go through the scalar data cache: JXLT_SCALAR_STORES_DONE() (s_dcache_wb) behind the last of
-// them writes it back -- the compiler does that at a kernel's end only for scalar stores of its own making.  Nothing
-// in the kernels READS these locations through the scalar cache.  (The CPU execution model: plain stores.)
-#ifndef JXLT_SCALAR_STORE64
-#define JXLT_SCALAR_STORE64(p, i, v) \
-  asm volatile("s_store_dwordx2 %0, %1, %2" ::"s"((unsigned long long)(v)), "s"(p), "n"((i) * 8) : "memory")
-// (Scalar memory operations complete out of order: the wait IN FRONT of s_dcache_wb is what makes it cover the stores
-// above it.  Without it the last stores of a wave could reach the cache behind the write-back and stay there, dirty,
-// until some later wave of those CUs wrote the cache back -- on a small frame nobody did before token_kernel read
-// the masks: one wrong context byte in two of six runs of the HDR tests, round 5.)
-#define JXLT_SCALAR_STORES_DONE() asm volatile("s_waitcnt lgkmcnt(0)\n\ts_dcache_wb\n\ts_waitcnt lgkmcnt(0)" ::: "memory")
-#endif
-
-// The same for a wave-uniform value in scalar registers (a pointer, an index).
+// JXLT_LAUNDER_VGPR for a wave-uniform value in scalar registers (a pointer, an index).
 #ifndef JXLT_LAUNDER_SGPR
 #define JXLT_LAUNDER_SGPR(x) asm volatile("" : "+s"(x))
 #endif

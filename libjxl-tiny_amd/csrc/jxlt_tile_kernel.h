@@ -1330,21 +1330,19 @@ JXLT_DI void tile_kernel_body(const TileArgs& A, const int tile_id) {
         // (1 << (covered - 1) is `covered` itself)
         m0[c] |= (unsigned long long)(uint32_t)__builtin_amdgcn_readfirstlane(nzeros <= 4 * covered ? covered : 0);
       }
-      // (the tokeniser takes "nonzeros still to come" and "previous coefficient nonzero" from these masks.  They are
-      // wave-uniform -- ballots, in scalar registers -- and leave by SCALAR stores: six s_store_dwordx2 to 48 contiguous
-      // bytes.  As vector stores by lanes 0 and 1 they cost eight vector instructions per channel: the scalar values
-      // moved to vector registers, selected per lane, a 64-bit address.)
-      // (scalar address arithmetic is not free here: in this phase every wave of the CU runs on the ONE scalar unit the
-      // four SIMDs share -- 462 scalar against 368 vector instructions per wave, round 5's per-phase counters --, so:
-      // one base per block with the channels at constant offsets, 32-bit products where the frame limit allows them
-      // (2^25 blocks * 48 bytes of masks), and nothing at all for the second block of a one-block transform.)
-      {
-        unsigned long long* masks = reinterpret_cast<unsigned long long*>(reinterpret_cast<char*>(A.blk_nzmask) + pos0 * 48u);
-        JXLT_LAUNDER_SGPR(masks);
+      // (the tokeniser takes "nonzeros still to come" and "previous coefficient nonzero" from these masks: six
+      // wave-uniform 64-bit values -- ballots, in scalar registers --, 48 contiguous bytes that lane 0 writes as three
+      // 16-byte stores off ONE scalar base.  They are ordinary vector stores on purpose: the scalar unit's way to memory
+      // is a cache of its own that the stores of nobody else go through, so it would have to be written back by hand.
+      // (The scalar address arithmetic is not free here: in this phase every wave of the CU runs on the ONE scalar unit
+      // the four SIMDs share -- so: one base per block with the channels at constant offsets, 32-bit products where the
+      // frame limit allows them (2^25 blocks * 48 bytes of masks), and nothing for the second block of a transform.)
+      if (lane == 0) {
+        unsigned long long* const masks = reinterpret_cast<unsigned long long*>(reinterpret_cast<char*>(A.blk_nzmask) + pos0 * 48u);
 #pragma unroll
         for (int c = 0; c < 3; c++) {
-          JXLT_SCALAR_STORE64(masks, 2 * c, m0[c]);
-          JXLT_SCALAR_STORE64(masks, 2 * c + 1, m1[c]);
+          masks[2 * c] = m0[c];
+          masks[2 * c + 1] = m1[c];
         }
       }
       {
@@ -1374,7 +1372,6 @@ JXLT_DI void tile_kernel_body(const TileArgs& A, const int tile_id) {
       if (next_b < 0) break;
       one_transform(set_b, set_a);
     }
-    JXLT_SCALAR_STORES_DONE();  // (the masks above: out of the scalar data cache)
     if (lane == 0 && wave_tokens) atomicAdd(&S.ntok, wave_tokens);
     if (kLutRoots) {
       if (__ballot(!(q_largest < 32768.0f)) != 0 && lane == 0) S.overflow = 1u;  // (suspect: see q_largest)

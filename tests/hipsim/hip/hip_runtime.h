@@ -414,8 +414,6 @@ typedef const float* JxltGlobalFloats;
 typedef int16_t* JxltGlobalShorts;
 typedef const int16_t* JxltGlobalConstShorts;
 typedef const uint32_t* JxltGlobalConstWords;
-#define JXLT_SCALAR_STORE64(p, i, v) ((p)[i] = (v))
-#define JXLT_SCALAR_STORES_DONE() ((void)0)
 #define JXLT_COMPILER_FENCE() ((void)0)
 typedef float4 JxltFloat4;  // (see jxlt_device_common.h: issue order and waits have no meaning here)
 #define JXLT_LDS_LOAD4_NOW(dst, p, byte_off) ((dst) = *reinterpret_cast<const float4*>(reinterpret_cast<const char*>(p) + (byte_off)))
