@@ -123,9 +123,10 @@ int jxlt_image_upload(jxlt_context* ctx, const float* const planes[3], size_t pi
  * ordinary memory).  Free with jxlt_pinned_free. */
 void* jxlt_pinned_alloc(size_t bytes);
 void jxlt_pinned_free(void* p);
-/* Page-locks memory the caller already owns (e.g. a shared-memory mapping that several processes assemble
- * one codestream in) so that the devices can copy from / to it directly.  Undo with jxlt_pinned_unregister
- * before the memory goes away. */
+/* Page-locks memory the caller already owns so that the devices can copy from / to it directly.  Undo with
+ * jxlt_pinned_unregister before the memory goes away.  Machines may refuse this for memory that already exists
+ * (JXLT_ERR_NO_DEVICE, nothing registered): take jxlt_pinned_alloc there, or leave the memory pageable where that is
+ * accepted.  The library itself registers nothing. */
 int jxlt_pinned_register(void* p, size_t bytes);
 void jxlt_pinned_unregister(void* p);
 
@@ -353,9 +354,10 @@ int jxlt_write_file_header(size_t xsize, size_t ysize, uint8_t** out_bytes, size
  * cut into rectangles of whole DC groups (2048 x 2048 pixels; jxlt_shard_rect), one per participant; every participant
  * runs the complete device pipeline on its slab with its own device context.  The only exchange is on the
  * host: the 2 x 64 x 64 symbol histograms are summed by participant 0, which builds the two prefix codes and
- * hands the code tables back; every participant then entropy-codes its sections on its GPU and copies them
- * straight into its byte range of ONE output buffer, where participant 0 writes frame header, TOC and the
- * global sections in front.  No device-to-device traffic, no RCCL.
+ * hands the code tables back; every participant then entropy-codes its sections on its GPU and puts them
+ * into its byte ranges of ONE output buffer (threads of one process: the device copies them straight there; one
+ * process per GPU: by way of the context's jxlt_output_buffer, the segment itself is never page-locked), where
+ * participant 0 writes frame header, TOC and the global sections in front.  No device-to-device traffic, no RCCL.
  *
  * Participants are host threads of one process (jxlt_multi_encoder_*, also behind jxl::EncodeFile when
  * jxl::SetEncoderDevices / JXLT_DEVICES names several GPUs) or one process per GPU that meet in a POSIX
@@ -403,7 +405,8 @@ void jxlt_shard_group_close(jxlt_shard_group* group);
 const char* jxlt_shard_group_last_error(const jxlt_shard_group* group);
 /* Collective over the group's ranks: `ctx` holds this rank's slab of an xsize x ysize frame (rows
  * jxlt_shard_rect(xsize, ysize, world, rank); jxlt_image_upload* / jxlt_image_set_device* with its width and height; ranks
- * with an empty range pass any context).  On rank 0 *bytes / *size receive the complete codestream (inside
+ * with an empty range pass any context).  The sections pass through ctx's jxlt_output_buffer: what it held is gone.
+ * On rank 0 *bytes / *size receive the complete codestream (inside
  * the segment, valid until the next encode); NULL / 0 on the other ranks. */
 int jxlt_shard_encode(jxlt_shard_group* group, jxlt_context* ctx, size_t xsize, size_t ysize, float distance,
                       const uint8_t** bytes, size_t* size);

@@ -85,7 +85,6 @@ struct jxlt_shard_group {
   int rank = 0;              // -1: in-process group (participants pass their rank explicitly)
   int world = 1;
   bool shm = false;
-  bool registered = false;   // output area page-locked for this process's devices
   bool unlinked = false;     // (rank 0) the segment's name is gone already
   std::string name;
   std::string error;         // first failure (several participants of one process may report)
@@ -448,7 +447,7 @@ int EncodeShard(jxlt_shard_group* g, int rank, const jxlt_slab_ops* ops, size_t 
   }
 
   stamp(5);
-  // ---- every participant's device writes its sections in place: a run of the codestream per row of the slab's
+  // ---- every participant's sections go to their places: a run of the codestream per row of the slab's
   // DC groups / groups (rows that follow each other in the frame's order -- a slab as wide as the frame -- are one run)
   uint8_t* out = g->output();
   std::vector<jxlt_section_run> dc_runs, ac_runs;
@@ -534,6 +533,66 @@ int CtxFinish(void* self) { return jxlt_synchronize(static_cast<jxlt_context*>(s
 
 jxlt_slab_ops OpsOf(jxlt_context* ctx) {
   return {ctx, CtxEnqueue, CtxDcHist, CtxBeginDc, CtxAcHist, CtxMeasure, CtxWrite, CtxFinish};
+}
+
+// ---- the same for an output area that the device cannot copy to directly: a segment shared with other processes is
+// ordinary memory to this process's GPU, and page-locking memory that already exists is something a machine may refuse.
+// The slab's sections leave the device for the context's own page-locked buffer (jxlt_output_buffer; DC groups, then AC
+// groups, back to back) and this thread puts them in their places once they are there.
+struct StagedSlab {
+  explicit StagedSlab(jxlt_context* c) : ctx(c) {}
+  jxlt_context* ctx;
+  jxlt_packed_sections dc = {nullptr, nullptr, nullptr, 0}, ac = {nullptr, nullptr, nullptr, 0};  // (of this frame)
+  const uint8_t* staged = nullptr;
+  uint8_t* out = nullptr;
+  const jxlt_section_run *dc_runs = nullptr, *ac_runs = nullptr;  // (EncodeShard's, alive until `finish`)
+  size_t n_dc = 0, n_ac = 0;
+};
+jxlt_context* CtxOf(void* self) { return static_cast<StagedSlab*>(self)->ctx; }
+size_t BytesOf(const jxlt_packed_sections& s) { return static_cast<size_t>(s.section_offset[s.num_sections]); }
+void PlaceRuns(const jxlt_packed_sections& s, const uint8_t* staged, uint8_t* out, const jxlt_section_run* runs, size_t n) {
+  for (size_t i = 0; i < n; ++i) {
+    const uint64_t lo = s.section_offset[runs[i].first_section];
+    const uint64_t hi = s.section_offset[runs[i].first_section + runs[i].num_sections];
+    memcpy(out + runs[i].dst_offset, staged + lo, hi - lo);
+  }
+}
+int StagedEnqueue(void* self, const jxlt_params* p) { return CtxEnqueue(CtxOf(self), p); }
+int StagedDcHist(void* self, const uint32_t** h) { return CtxDcHist(CtxOf(self), h); }
+int StagedBeginDc(void* self, const uint32_t* t) { return CtxBeginDc(CtxOf(self), t); }
+int StagedAcHist(void* self, const uint32_t** h) { return CtxAcHist(CtxOf(self), h); }
+int StagedMeasure(void* self, const uint32_t* t, jxlt_packed_sections* dc, jxlt_packed_sections* ac) {
+  StagedSlab* slab = static_cast<StagedSlab*>(self);
+  const int rc = CtxMeasure(slab->ctx, t, dc, ac);
+  slab->dc = *dc;
+  slab->ac = *ac;
+  return rc;
+}
+int StagedWrite(void* self, uint8_t* out, const jxlt_section_run* dc_runs, size_t n_dc, const jxlt_section_run* ac_runs,
+                size_t n_ac) {
+  StagedSlab* slab = static_cast<StagedSlab*>(self);
+  uint8_t* staged = nullptr;
+  int rc = jxlt_output_buffer(slab->ctx, BytesOf(slab->dc) + BytesOf(slab->ac) + 16, &staged);
+  if (rc == JXLT_OK) rc = jxlt_pack_deliver(slab->ctx, 0, staged, nullptr, 0, 0);
+  if (rc == JXLT_OK) rc = jxlt_pack_deliver(slab->ctx, 1, staged + BytesOf(slab->dc), nullptr, 0, 0);
+  slab->staged = staged;
+  slab->out = out;
+  slab->dc_runs = dc_runs;
+  slab->n_dc = n_dc;
+  slab->ac_runs = ac_runs;
+  slab->n_ac = n_ac;
+  return rc;
+}
+int StagedFinish(void* self) {
+  StagedSlab* slab = static_cast<StagedSlab*>(self);
+  const int rc = CtxFinish(slab->ctx);
+  if (rc != JXLT_OK) return rc;
+  PlaceRuns(slab->dc, slab->staged, slab->out, slab->dc_runs, slab->n_dc);
+  PlaceRuns(slab->ac, slab->staged + BytesOf(slab->dc), slab->out, slab->ac_runs, slab->n_ac);
+  return JXLT_OK;
+}
+jxlt_slab_ops OpsOf(StagedSlab* slab) {
+  return {slab, StagedEnqueue, StagedDcHist, StagedBeginDc, StagedAcHist, StagedMeasure, StagedWrite, StagedFinish};
 }
 
 size_t SectionsOf(size_t xsize, size_t ysize) {
@@ -905,7 +964,6 @@ int jxlt_shard_group_open(const char* shm_name, int rank, int world, size_t outp
 
 void jxlt_shard_group_close(jxlt_shard_group* g) {
   if (!g) return;
-  if (g->registered) jxlt_pinned_unregister(g->output());
   if (g->shm) {
     munmap(g->base, g->bytes);
     if (g->rank == 0 && !g->unlinked) shm_unlink(g->name.c_str());
@@ -959,13 +1017,8 @@ int jxlt_shard_encode(jxlt_shard_group* g, jxlt_context* ctx, size_t xsize, size
       if (restore) (void)sched_setaffinity(0, sizeof(saved), &saved);
     }
   } near_device(jxlt_context_device(ctx));
-  if (!g->registered) {
-    // the devices copy their sections straight into the segment: page-lock this process's mapping of it
-    if (jxlt_pinned_register(g->output(), static_cast<size_t>(g->ctl->output_capacity)) != JXLT_OK)
-      return jxlt::Fail(g, JXLT_ERR_NO_DEVICE, "cannot page-lock the shared output area");
-    g->registered = true;
-  }
-  const jxlt_slab_ops ops = jxlt::OpsOf(ctx);
+  jxlt::StagedSlab slab(ctx);
+  const jxlt_slab_ops ops = jxlt::OpsOf(&slab);
   return jxlt::EncodeShard(g, g->rank, &ops, xsize, ysize, distance, bytes, size);
 }
 
