@@ -9,6 +9,13 @@
 #include <cstdint>
 #include <cstdio>
 
+// (no packed FP32 arithmetic in the kernel, whatever flags it is built with: some of its forms have given wrong results)
+#ifdef __HIP_DEVICE_COMPILE__
+#define NO_PACKED_FP32 __attribute__((target("no-packed-fp32-ops")))
+#else
+#define NO_PACKED_FP32
+#endif
+
 __device__ __forceinline__ float div_normal(float num, float den) {
   const float r0 = __builtin_amdgcn_rcpf(den);
   const float e0 = __builtin_fmaf(-den, r0, 1.0f);
@@ -30,7 +37,7 @@ __device__ __forceinline__ float pick(uint32_t h) {
   return __uint_as_float((e << 23) | (h & 0x7FFFFFu));
 }
 
-__global__ void probe(unsigned long long* bad, unsigned long long* bad_rcp, uint32_t seed) {
+NO_PACKED_FP32 __global__ void probe(unsigned long long* bad, unsigned long long* bad_rcp, uint32_t seed) {
   const uint32_t i = blockIdx.x * blockDim.x + threadIdx.x;
   unsigned long long b = 0, br = 0;
   for (uint32_t k = 0; k < 1024; k++) {

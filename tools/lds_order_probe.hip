@@ -6,8 +6,15 @@
 #include <cstdio>
 #include <vector>
 
+// (no packed FP32 arithmetic in the kernel, whatever flags it is built with: some of its forms have given wrong results)
+#ifdef __HIP_DEVICE_COMPILE__
+#define NO_PACKED_FP32 __attribute__((target("no-packed-fp32-ops")))
+#else
+#define NO_PACKED_FP32
+#endif
+
 template <int VARIANT, bool WAIT>
-__global__ void probe(const float* in, float* out, int iters) {
+NO_PACKED_FP32 __global__ void probe(const float* in, float* out, int iters) {
   __shared__ float lds[64 * 72 * 2];
   const int tid = threadIdx.x, l = tid & 7, oct = tid >> 3;
   float* sc = lds + oct * 72;

@@ -12,8 +12,14 @@
   asm volatile(STR : "+v"(y[10]) : "v"(a), "v"(b), "v"(y[9])); asm volatile(STR : "+v"(y[11]) : "v"(a), "v"(b), "v"(y[10])); \
   asm volatile(STR : "+v"(y[12]) : "v"(a), "v"(b), "v"(y[11])); asm volatile(STR : "+v"(y[13]) : "v"(a), "v"(b), "v"(y[12])); \
   asm volatile(STR : "+v"(y[14]) : "v"(a), "v"(b), "v"(y[13])); asm volatile(STR : "+v"(y[15]) : "v"(a), "v"(b), "v"(y[14]));
+// (no packed FP32 arithmetic in the kernel, whatever flags it is built with: some of its forms have given wrong results)
+#ifdef __HIP_DEVICE_COMPILE__
+#define NO_PACKED_FP32 __attribute__((target("no-packed-fp32-ops")))
+#else
+#define NO_PACKED_FP32
+#endif
 template <int MODE>
-__global__ void __launch_bounds__(256) k(float* out, int iters, float a, float b) {
+NO_PACKED_FP32 __global__ void __launch_bounds__(256) k(float* out, int iters, float a, float b) {
   asm volatile("s_mov_b64 s[20:21], 0x33333333" ::: "s20", "s21");
   float y[16];
   for (int i = 0; i < 16; i++) y[i] = threadIdx.x * 0.003f + i + 1.0f;

@@ -14,7 +14,7 @@
 // stream at the same time: W / 2 workgroups of 512 threads -- tile_kernel's shape -- are pinned on every CU by
 // their LDS footprint; `overlap` reports which share of the kernel's span had every wave in flight).
 //
-// build: hipcc --offload-arch=gfx950 -O2 -o tools/valu_issue_probe tools/valu_issue_probe.hip
+// build: hipcc --offload-arch=gfx950 -O2 -Xclang -target-feature -Xclang -packed-fp32-ops -o tools/valu_issue_probe tools/valu_issue_probe.hip
 #include <hip/hip_runtime.h>
 #include <cstdio>
 #include <cstdlib>
@@ -37,7 +37,6 @@ enum Mode {
   MUL,            // v_mul_f32 vN, vN, v48          (VOP2)
   ADD,            // v_add_f32 vN, vN, v48
   MOV,            // v_mov_b32 vN, v48
-  PK_FMA,         // v_pk_fma_f32 v[N:N+1], v[N:N+1], v[48:49], v[50:51]  (8 instructions = 16 lanes-ops)
   CHAIN1,         // v_fma_f32 v32, v32, v48, v49   ONE dependent chain (dependent-issue latency)
   CHAIN2,         // two chains
   CHAIN4,         // four chains
@@ -69,7 +68,7 @@ enum Mode {
 static const char* kModeNames[NUM_MODES] = {
     "v_fma_f32 3 VGPR sources, distinct", "v_fma_f32 3 VGPR sources, same bank", "v_fma_f32 one VGPR three times",
     "v_fma_f32 with SGPR source", "v_mul_f32 with 32-bit literal", "v_fma_f32 with inline constant",
-    "v_fmac_f32 (VOP2)", "v_mul_f32 (VOP2)", "v_add_f32 (VOP2)", "v_mov_b32", "v_pk_fma_f32 (2 fma per lane)",
+    "v_fmac_f32 (VOP2)", "v_mul_f32 (VOP2)", "v_add_f32 (VOP2)", "v_mov_b32",
     "v_fma_f32 1 dependent chain", "v_fma_f32 2 chains", "v_fma_f32 4 chains", "fma/mul/add/fmac mix, 16 chains",
     "v_cndmask_b32_e64 SGPR mask", "v_max_f32", "v_rndne_f32", "v_mul_f32 with SGPR source (VOP2)",
     "v_mul_f32_e64 with neg modifier", "v_fma_f32 with neg modifier", "v_sub_f32", "v_min_f32", "v_cmp_gt_f32 -> vcc",
@@ -142,12 +141,6 @@ __global__ void __launch_bounds__(512) probe(unsigned long long* cycles, float* 
                    "v_rndne_f32 v36, v36\n\t v_rndne_f32 v37, v37\n\t v_rndne_f32 v38, v38\n\t v_rndne_f32 v39, v39\n\t"
                    "v_rndne_f32 v40, v40\n\t v_rndne_f32 v41, v41\n\t v_rndne_f32 v42, v42\n\t v_rndne_f32 v43, v43\n\t"
                    "v_rndne_f32 v44, v44\n\t v_rndne_f32 v45, v45\n\t v_rndne_f32 v46, v46\n\t v_rndne_f32 v47, v47" CLOB);
-    }
-    if (MODE == PK_FMA) {
-      asm volatile(REP4("v_pk_fma_f32 v[32:33], v[32:33], v[48:49], v[50:51]\n\t"
-                        "v_pk_fma_f32 v[34:35], v[34:35], v[48:49], v[50:51]\n\t"
-                        "v_pk_fma_f32 v[36:37], v[36:37], v[48:49], v[50:51]\n\t"
-                        "v_pk_fma_f32 v[38:39], v[38:39], v[48:49], v[50:51]\n\t") CLOB);
     }
     if (MODE == CHAIN1) { asm volatile(REP16("v_fma_f32 v32, v32, v48, v49\n\t") CLOB); }
     if (MODE == CHAIN2) {
@@ -282,7 +275,6 @@ int main(int argc, char** argv) {
   run_all<MUL>(d_cycles, d_sink, json, &first, false);
   run_all<ADD>(d_cycles, d_sink, json, &first, false);
   run_all<MOV>(d_cycles, d_sink, json, &first, false);
-  run_all<PK_FMA>(d_cycles, d_sink, json, &first, true);
   run_all<CHAIN1>(d_cycles, d_sink, json, &first, true);
   run_all<CHAIN2>(d_cycles, d_sink, json, &first, false);
   run_all<CHAIN4>(d_cycles, d_sink, json, &first, true);
