@@ -858,9 +858,9 @@ JXLT_DI void tile_kernel_body(const TileArgs& A, const int tile_id) {
       // (issued HERE, a round ahead of their use: as plain loads the compiler sinks them to their first use behind the
       // loop's exit test and every round waits for the LDS -- JXLT_LDS_LOAD4_NOW, jxlt_device_common.h)
       // (addresses in integers that move on by a round -- 4 KB -- per request: two additions.  No clamp at the end of
-      // the tile: what the last requests fetch is never used -- with an even number of rounds one round beyond the
-      // terms, with an odd number two, i.e. never more than 4 KB beyond the term area's 64 blocks --, and those 4 KB lie
-      // inside the workgroup's LDS: the transposes' pad, static_assert below.)
+      // the tile: with an even number of rounds the last request goes one round beyond the terms and is never used, i.e.
+      // never more than 4 KB beyond the term area's 64 blocks, and those 4 KB lie inside the workgroup's LDS: the
+      // transposes' pad, static_assert below.)
       auto a1 = JXLT_LDS_ADDRESS(first_factors) + (decltype(JXLT_LDS_ADDRESS(first_factors)))(relay_pos << 10);
       auto a2 = JXLT_LDS_ADDRESS(second_factors) + (decltype(a1))(relay_pos << 10);
       static_assert(offsetof(TileShared, x) + (size_t)kCflTermFloats * 4 + 4 * 1024 <= sizeof(TileShared),
@@ -897,9 +897,8 @@ JXLT_DI void tile_kernel_body(const TileArgs& A, const int tile_id) {
         vdst = __uint_as_float(r[0]);
         src0 = __uint_as_float(r[1]);
       };
-      // one round: the set `t` has arrived when all but the four loads of the OTHER set, requested behind it, have
+      // one round, of a set that has arrived
       auto round4 = [&](JxltFloat4* t) {
-        JXLT_LDS_WAIT4(4, t[0], t[1], t[2], t[3]);
         block_steps(acc, t);   // row 0
         hop16(acc2, acc);      // acc row 0 -> acc2 row 1
         block_steps(acc2, t);  // row 1
@@ -909,17 +908,21 @@ JXLT_DI void tile_kernel_body(const TileArgs& A, const int tile_id) {
         block_steps(acc2, t);  // row 2
         hop32(acc2, acc);      // acc2 row 2 -> acc row 0
       };
+      // (two rounds at a time.  A set has arrived when all but the four loads of the OTHER set, requested behind it, have.
+      // The odd round at the end stands behind the loop: inside it, as a round that is skipped, the loop had a path -- one
+      // that no tile takes -- back to a request into registers that the skipped round's loads were still on their way to)
       request(ta);
 #pragma clang loop unroll(disable)
-      for (int blk = 0; blk < nblk_pad; blk += 8) {
+      for (int blk = 4; blk < nblk_pad; blk += 8) {
         request(tb);
+        JXLT_LDS_WAIT4(4, ta[0], ta[1], ta[2], ta[3]);
         round4(ta);
         request(ta);
-        if (blk + 4 < nblk_pad) round4(tb);  // (wave-uniform: an odd number of rounds ends here)
+        JXLT_LDS_WAIT4(4, tb[0], tb[1], tb[2], tb[3]);
+        round4(tb);
       }
-      // (whatever was requested last is not used; it has arrived before its registers serve anything else)
-      JXLT_LDS_DRAIN4(ta[0], ta[1], ta[2], ta[3]);
-      JXLT_LDS_DRAIN4(tb[0], tb[1], tb[2], tb[3]);
+      JXLT_LDS_WAIT4(0, ta[0], ta[1], ta[2], ta[3]);  // (an even number of rounds: not used, but arrived)
+      if (nblk_pad & 4) round4(ta);  // (wave-uniform)
       JXLT_DEFINE_VGPR(late_root0);
       JXLT_DEFINE_VGPR(late_root1);
       JXLT_DEFINE_VGPR(late_zeros_cost);

@@ -420,7 +420,6 @@ typedef float4 JxltFloat4;  // (see jxlt_device_common.h: issue order and waits 
 #define JXLT_LDS_ADDRESS(p) ((uintptr_t)(p))  // (no separate LDS address space here: the pointer itself)
 #define JXLT_LDS_LOAD4_NOW_AT(dst, addr, byte_off) ((dst) = *reinterpret_cast<const float4*>((addr) + (byte_off)))
 #define JXLT_LDS_WAIT4(n, a, b, c, d) ((void)0)
-#define JXLT_LDS_DRAIN4(a, b, c, d) ((void)0)
 #define JXLT_STORES_WRITTEN() ((void)0)
 
 // v_rcp_f32 (1 ulp on hardware; the model returns the correctly rounded reciprocal)
