@@ -508,12 +508,14 @@ int jxlt_pinned_register(void* p, size_t bytes) {
   return JXLT_OK;
 }
 
+// (neither reports a failure, so neither may leave one for the next launch check of this thread to find: a caller
+// whose registration was refused cleans up all the same)
 void jxlt_pinned_unregister(void* p) {
-  if (p) (void)hipHostUnregister(p);
+  if (p && hipHostUnregister(p) != hipSuccess) (void)hipGetLastError();
 }
 
 void jxlt_pinned_free(void* p) {
-  if (p) (void)hipHostFree(p);
+  if (p && hipHostFree(p) != hipSuccess) (void)hipGetLastError();
 }
 
 int jxlt_image_set_device(jxlt_context* ctx, const void* const device_planes[3], size_t pitch_bytes,
