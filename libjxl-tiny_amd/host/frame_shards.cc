@@ -920,8 +920,12 @@ int jxlt_shard_group_open(const char* shm_name, int rank, int world, size_t outp
   if (rank == 0) {
     shm_unlink(shm_name);  // a stale segment of a run that died
     fd = shm_open(shm_name, O_CREAT | O_EXCL | O_RDWR, 0600);
-    if (fd < 0 || ftruncate(fd, static_cast<off_t>(bytes)) != 0) {
-      if (fd >= 0) close(fd);
+    if (fd < 0) return JXLT_ERR_OUT_OF_MEMORY;
+    // (room for the whole segment now: a segment that is only sized takes its pages when they are first written, and a
+    // rank that writes its sections when the shared-memory file system has none left is killed by a signal)
+    if (ftruncate(fd, static_cast<off_t>(bytes)) != 0 || posix_fallocate(fd, 0, static_cast<off_t>(bytes)) != 0) {
+      close(fd);
+      shm_unlink(shm_name);
       return JXLT_ERR_OUT_OF_MEMORY;
     }
   } else {

@@ -18,6 +18,21 @@ def test_the_host_library_page_locks_nothing_that_it_does_not_own(built):
     assert "jxlt_pinned_register" not in wanted and "HostRegister" not in wanted
 
 
+def test_a_segment_that_the_file_system_has_no_room_for_is_refused(built):
+    """... when it is opened, not by a signal when somebody's sections reach a page that is not there."""
+    fs = os.statvfs("/dev/shm")
+    if fs.f_blocks == 0:
+        pytest.skip("/dev/shm has no limit here")
+    name = "/jxlt-no-room-%d" % os.getpid()
+    with pytest.raises(built.JxlTinyError):
+        built.ShardGroup(name, 0, 2, fs.f_blocks * fs.f_frsize + (1 << 30), 4096)
+    assert not os.path.exists("/dev/shm" + name)
+    grp = built.ShardGroup(name, 0, 1, 1 << 20, 4096)
+    segment = os.stat("/dev/shm" + name)
+    assert segment.st_size > 1 << 20 and segment.st_blocks * 512 >= segment.st_size  # (every page is there)
+    grp.close()
+
+
 def _slab(planes, rect):
     x0, y0, x1, y1 = rect
     return np.ascontiguousarray(planes[:, y0:y1, x0:x1])
