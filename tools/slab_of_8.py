@@ -155,8 +155,8 @@ def main():
            "same_bytes_as_single_gpu": bool(same), "errors": errors,
            "note": "serial stage + hand-over = ms_per_frame_median - kernels; the seven replaying participants are native threads "
                    "(tools/slab_replay.cc; round 5: Python threads taking turns on the interpreter lock); the peers answer at once, so nothing here is waiting for a slower "
-                   "GPU; every participant's section bytes land in one shared output buffer (participant 0's by DMA from the GPU, the "
-                   "others' by memcpy)"}
+                   "GPU; every participant's section bytes land in one shared output buffer (participant 0's from the GPU by way of "
+                   "its context's page-locked buffer, the others' by memcpy)"}
     line = json.dumps(doc)
     print(line)
     if out_path:
