@@ -171,11 +171,10 @@ def test_values_outside_unit_range(enc):
 
 
 def test_small_frames_give_the_same_tokens_every_time(enc):
-    """The nonzero masks leave tile_kernel by scalar stores through the scalar data cache (jxlt_device_common.h:
-    JXLT_SCALAR_STORE64 / JXLT_SCALAR_STORES_DONE).  On a frame of a few tiles nothing but the kernel's own
-    write-back puts them in memory before token_kernel reads them: with the write-back issued ahead of the stores it
-    was meant to cover (scalar memory operations complete out of order) one context byte in this frame's 26 578
-    records was wrong in about every third run (round 5).  Sixty runs here."""
+    """token_kernel reads what tile_kernel stored -- coefficients and the nonzero masks -- right behind it.  On a frame of
+    a few tiles nothing but the order of the two kernels puts those stores in memory in time: when the masks went
+    through a cache that had to be written back by hand, and the write-back could overtake them, one context byte in
+    this frame's 26 578 records was wrong in about every third run.  Sixty runs here."""
     rng = np.random.default_rng(7)
     planes = (rng.random((3, 72, 136)) * 3.0 - 1.0).astype(np.float32)  # the frame of test_values_outside_unit_range
     want = T.oracle_hot_path(planes, 1.0)
@@ -546,8 +545,8 @@ def _shard_rank(rank, world, name, w, h, d, q, barrier):
 
 def test_shard_group_two_processes_on_one_gpu(built):
     """jxlt_shard_group_* / jxlt_shard_encode: the one-process-per-GPU form bench.py's ranks use -- two
-    processes (both on GPU 0 here), the output area in POSIX shared memory page-locked by each of them,
-    each process's GPU copying its sections straight into it."""
+    processes (both on GPU 0 here), the output area in POSIX shared memory, each process's sections going there
+    by way of its context's page-locked buffer."""
     import multiprocessing as mp
     import os
     w, h, d = 600, 2048 + 520, 2.0
